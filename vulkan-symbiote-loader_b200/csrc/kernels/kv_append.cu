@@ -138,9 +138,13 @@ __global__ void __launch_bounds__(KA_THREADS) vsl_kv_append_kernel(KvAppendParam
         bad = true;
     }
     if (bad && threadIdx.x == 0) set_status(p.status, VSL_ERR_BOUNDS);
-    if (page < 0) {
+    if (page < 0) {  // the CTA's row: zeros as they are, for a norm or rotation may make NaN of them
 #pragma unroll
-        for (int i = 0; i < HEADS; i++) x[i][0] = x[i][1] = x[i][2] = x[i][3] = 0.0f;
+        for (int i = 0; i < HEADS; i++)
+            if (h_first + i < p.n_heads)
+                __stcs(reinterpret_cast<float4*>(p.q_out + ((size_t)r * p.n_heads + h_first + i) * HD) + sl,
+                       make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+        return;
     }
     if (p.q_norm || p.k_norm) {
         float mine = 0.0f;
@@ -169,7 +173,7 @@ __global__ void __launch_bounds__(KA_THREADS) vsl_kv_append_kernel(KvAppendParam
         }
     }
     if (p.cos) {
-        const size_t row = page >= 0 ? (size_t)pos * (HD / 2) : 0;
+        const size_t row = (size_t)pos * (HD / 2);
         if (p.halves) {
             const float4 c = __ldg(reinterpret_cast<const float4*>(p.cos + row) + sl % (L / 2));
             const float4 d = __ldg(reinterpret_cast<const float4*>(p.sin + row) + sl % (L / 2));
@@ -205,7 +209,7 @@ __global__ void __launch_bounds__(KA_THREADS) vsl_kv_append_kernel(KvAppendParam
     if (KVDT == VSL_Q4_0 && __any_sync(0xffffffffu, h_first + HEADS > p.n_heads)) q4_codes<HEADS>(x, codes, d);
     const size_t head_bytes = kv_head_page_bytes(KVDT, HD, p.page_size);
     // head 0 of K and of V in the row's page, and the lane's place in a head
-    const size_t page_at = page >= 0 ? (size_t)page * p.n_kv * head_bytes : 0;
+    const size_t page_at = (size_t)page * p.n_kv * head_bytes;
     const int b = sl >> 3, u = sl & 7;
     const size_t k_at = page_at + (KVDT == VSL_Q4_0 ? kv_q4_k_piece(NB, slot, b, u) : ((size_t)slot * HD + 4 * sl) * (KVDT == VSL_F16 ? 2 : 4));
     const size_t v_at = KVDT == VSL_Q4_0 ? page_at + kv_q4_v_piece(NB, slot, b, u) : k_at;
@@ -214,12 +218,11 @@ __global__ void __launch_bounds__(KA_THREADS) vsl_kv_append_kernel(KvAppendParam
     for (int i = 0; i < HEADS; i++) {
         const int h = h_first + i;
         if (h >= H) continue;
-        if (h < p.n_heads) {  // a padding or refused row gives zeros
+        if (h < p.n_heads) {
             __stcs(reinterpret_cast<float4*>(p.q_out + ((size_t)r * p.n_heads + h) * HD) + sl,
                    make_float4(x[i][0], x[i][1], x[i][2], x[i][3]));
             continue;
         }
-        if (page < 0) continue;
         const bool is_v = h >= p.n_heads + p.n_kv;
         unsigned char* cache = (is_v ? p.v_cache : p.k_cache) + (size_t)(h - p.n_heads - (is_v ? p.n_kv : 0)) * head_bytes;
         unsigned char* dst = cache + (is_v ? v_at : k_at);
