@@ -255,9 +255,10 @@ VSL_API int vsl_kv_read(const void* k_cache, const void* v_cache, int kvdtype, i
  * (query head h reads KV head h * n_kv / n_heads). A row at a negative position sees nothing and
  * gives zeros. Positions past max_pages * page_size and pages outside [0, n_pages) are not read;
  * status (nullable device int) then receives VSL_ERR_BOUNDS. Masked positions may hold anything,
- * NaN included. Sums and statistics are fp32; errors are those of fp32 arithmetic, but a weight's not
- * below 2^-50 of the row's largest weight, and with many rows a value's not below 2^-33 of the largest
- * one near it (64 positions). B <= 1024. workspace: vsl_flash_decode_q4_workspace_size bytes, 16-byte aligned,
+ * NaN included. Sums and statistics are fp32; errors are those of fp32 arithmetic, weights down to
+ * 2^-50 of the row's largest (few rows: a weight times its V scale, down to 2^-50 of the largest weight
+ * times the largest V scale read), and with many rows values down to 2^-33 of the largest one near them
+ * (64 positions). B <= 1024. workspace: vsl_flash_decode_q4_workspace_size bytes, 16-byte aligned,
  * zero-filled before its first use (its counters are left zero by every call); calls of different
  * shapes may share one sized for the largest, in the order of one stream. Results do not depend on
  * timing. One launch. */

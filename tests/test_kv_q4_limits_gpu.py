@@ -1,8 +1,12 @@
-"""4-bit KV cache on the GPU at the ends of its ranges."""
+"""4-bit KV cache on the GPU at the ends of its ranges: padding rows whatever the norm, weights and values
+far below the largest. The documented errors of the attention are those of fp32 arithmetic, with few rows
+for a weight times its V scale down to 2^-50 of the row's largest weight times the largest scale read."""
+import numpy as np
 import pytest
 
+import kv_q4_ref as R
 import vsl
-from test_kv_q4_gpu import Cache, dev, rope_tables
+from test_kv_q4_gpu import Cache, dev, rope_tables, status_word
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -31,3 +35,83 @@ def test_padding_rows_are_zero_whatever_the_norm(kvdt, hd, style, n):
         q = c.append(x, nh, *norms, seq, pad + 129, cos, sin, style, eps=0.0)  # past the table
         assert (q == 0).all() and c.status.item() == -5
     assert torch.equal(c.k, before[0]) and torch.equal(c.v, before[1])
+
+
+def values(codes, sc):
+    """codes [2, pages, nkv, page, hd], scales [2, pages, nkv, page, hd / 32] -> K, V float64 [nkv, len, hd]."""
+    with np.errstate(invalid="ignore"):
+        x = (codes.astype(np.float64) - 8) * np.repeat(sc.astype(np.float64), 32, -1)
+    return x.transpose(0, 2, 1, 3, 4).reshape(2, codes.shape[2], -1, codes.shape[-1])
+
+
+def attend(q, codes, sc, pos, mask=None):
+    """q fp32 [rows, nh, hd] of one sequence whose pages are codes, sc in order; status has to stay 0."""
+    (rows, nh, hd), (_, pages, nkv, page, _) = q.shape, codes.shape
+    kc, vc = (dev(R.pack(codes[i], sc[i], page, bool(i))) for i in range(2))
+    out, st = torch.full((rows, nh, hd), 7.0, device="cuda"), status_word()
+    n = vsl.flash_decode_q4_workspace_size(1, rows, nh, nkv, hd)
+    ws = torch.zeros(n, dtype=torch.uint8, device="cuda")
+    vsl.flash_decode_q4(dev(q), kc, vc, pages, dev(np.arange(pages, dtype=np.int32)[None]), pages, page,
+                        dev(np.array([pos], np.int32)), 1, rows, nh, nkv, hd, out, ws, n, sparse=mask, status=st)
+    assert st.item() == 0
+    return out.cpu().numpy().astype(np.float64)
+
+
+def floor_of(q, codes, sc, pos):
+    """What the documented limit of 2^-50 adds to an element's error: [rows, nh, hd]."""
+    k, _ = values(codes, sc)
+    rows, nh, hd = q.shape
+    nkv = k.shape[0]
+    out = np.zeros((rows, nh, hd))
+    for r in range(rows):
+        n = pos + r + 1
+        for h in range(nh):
+            g = h * nkv // nh
+            s = k[g, :n] @ q[r, h].astype(np.float64) / np.sqrt(hd)
+            w = np.exp(s - s.max())
+            top = np.abs(sc[1].astype(np.float64)[:, g]).max()
+            c = np.abs(codes[1][:, g].reshape(-1, hd)[:n].astype(np.float64) - 8).sum(0)
+            out[r, h] = 2.0 ** -50 * (w / w.sum()).max() * top * c
+    return out
+
+
+def random_cache(rng, pages, nkv, hd, k_scale=0.2, v_scale=0.2, page=64):
+    codes = rng.integers(0, 16, (2, pages, nkv, page, hd)).astype(np.uint8)
+    sc = rng.standard_normal((2, pages, nkv, page, hd // 32))
+    sc[0] *= k_scale
+    sc[1] *= v_scale
+    return codes, sc.astype(np.float16)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh,nkv", [(2, 2), (8, 2), (8, 1)])
+@pytest.mark.parametrize("k", [24, 28, 36, 42])
+def test_weights_far_below_the_largest(hd, nh, nkv, k):
+    """The first position has all the weight and the value 0: the output is what the others, of weights
+    around 2^-k, add up to."""
+    rng = np.random.default_rng(hd + nh + nkv + k)
+    codes, sc = random_cache(rng, 5, nkv, hd, k_scale=0.01)
+    codes[0, 0, :, 0], sc[0, 0, :, 0] = 15, np.float16(k * np.log(2) / (7 * np.sqrt(hd)))
+    codes[1, 0, :, 0] = 8
+    q = (1 + 0.1 * rng.standard_normal((1, nh, hd))).astype(np.float32)
+    got = attend(q, codes, sc, 299)
+    kk, vv = values(codes, sc)
+    want, tol = R.attention(q.astype(np.float64), kk[:, :300], vv[:, :300], 299)
+    tol += floor_of(q, codes, sc, 299)
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh,nkv", [(2, 2), (8, 2), (8, 1)])
+@pytest.mark.parametrize("r", [20, 30])
+def test_a_block_of_much_larger_values(hd, nh, nkv, r):
+    """One block's V scales are 2^r times another's."""
+    rng = np.random.default_rng(hd + nh + nkv + r)
+    codes, sc = random_cache(rng, 5, nkv, hd, v_scale=2.0 ** -15)
+    sc[1, ..., 0] = (rng.standard_normal(sc[1, ..., 0].shape) * 2.0 ** (r - 17)).astype(np.float16)
+    q = rng.standard_normal((1, nh, hd)).astype(np.float32)
+    got = attend(q, codes, sc, 299)
+    kk, vv = values(codes, sc)
+    want, tol = R.attention(q.astype(np.float64), kk[:, :300], vv[:, :300], 299)
+    tol += floor_of(q, codes, sc, 299)
+    assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())

@@ -128,15 +128,18 @@ __device__ __forceinline__ uint32_t hmax_abs2(uint32_t a, uint32_t b) {
     asm("max.xorsign.abs.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
     return r;
 }
+// the two halves of h times k (fp16), plus c, in fp32
+__device__ __forceinline__ float2 fma_half(uint32_t h, unsigned short k, float2 c) {
+    float2 r;
+    asm("{.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tfma.rn.f32.f16 %0, a, %3, %4;\n\tfma.rn.f32.f16 %1, b, %3, %5;}"
+        : "=f"(r.x), "=f"(r.y)
+        : "r"(h), "h"(k), "f"(c.x), "f"(c.y));
+    return r;
+}
 // transpose of an 8x8 matrix of fp16 (row lane / 4, columns 2 (lane % 4) and + 1)
 __device__ __forceinline__ uint32_t transpose8(uint32_t a) {
     uint32_t r;
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_rz(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
 
@@ -459,7 +462,10 @@ __global__ void __launch_bounds__(FQ_THREADS, FQ_CTAS_PER_SM) vsl_flash_decode_q
         l = make_float2(0.0f, 0.0f);                     // sums over this lane's positions
         uint32_t d_exp = 103;                            // largest exponent of a V scale so far (2^-24 at least)
         f = __uint_as_float((127u + 16u + 24u) << 23);   // 2^16 / 2^(d_exp - 127): d f is at most 65504
-        const uint32_t lo_mask = SPLIT_N && t4 >= 2 ? 0xffffe000u : 0u;
+        // SPLIT_N: columns 0-3 take p d rounded to fp16, columns 4-7 the rest, 2^11 times as large, as without the
+        // factor it would end at fp16's 2^-24, a part of 2^-40 of the largest
+        const float2 low_scale = t4 >= 2 ? make_float2(2048.0f, 2048.0f) : make_float2(1.0f, 1.0f);
+        const unsigned short low_take = t4 >= 2 ? 0xe800 : 0;  // -2048, 0
 
         // adds the earlier chains' sums to the accumulators
         float2 chain_m = mc;   // mc and f at the end of the last chain
@@ -634,10 +640,9 @@ __global__ void __launch_bounds__(FQ_THREADS, FQ_CTAS_PER_SM) vsl_flash_decode_q
                             if (pf[hf].y == 0.0f) pd.y = 0.0f;
                         }
                         if (SPLIT_N) {
-                            const float2 t = make_float2(__uint_as_float(__float_as_uint(pd.x) & lo_mask),
-                                                         __uint_as_float(__float_as_uint(pd.y) & lo_mask));
-                            pd = fma2(t, make_float2(-1.0f, -1.0f), pd);
-                            bh[hf] = transpose8(pack_rz(pd.x, pd.y));
+                            const uint32_t hi = pack_rn(pd.x, pd.y);
+                            const float2 r = fma_half(hi, low_take, mul2(pd, low_scale));
+                            bh[hf] = transpose8(pack_rn(r.x, r.y));
                         } else {
                             const uint32_t hi = pack_rn(pd.x, pd.y);
                             const float2 t = make_float2(half_lo(hi), half_hi(hi));
@@ -695,13 +700,17 @@ __global__ void __launch_bounds__(FQ_THREADS, FQ_CTAS_PER_SM) vsl_flash_decode_q
         add_chains();
 
         // ---- the segment's result: lane (g4, t4) holds columns 2 t4, + 1, dimensions 32 i + 4 g4 .. + 3 ----
-        if (SPLIT_N) {  // columns 4-7 hold the low parts of 0-3
+        if (SPLIT_N) {  // columns 4-7 hold the low parts of 0-3, times 2^11
+            const float unit = t4 >= 2 ? 1.0f / 2048.0f : 1.0f;
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
                 for (int j = 0; j < 2; j++)
 #pragma unroll
-                    for (int k = 0; k < 4; k++) o[i][j][k] += __shfl_xor_sync(0xffffffffu, o[i][j][k], 2);
+                    for (int k = 0; k < 4; k++) {
+                        o[i][j][k] *= unit;
+                        o[i][j][k] += __shfl_xor_sync(0xffffffffu, o[i][j][k], 2);
+                    }
         }
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) {
