@@ -1,6 +1,7 @@
 """4-bit KV cache on the GPU at the ends of its ranges: padding rows whatever the norm, weights and values
-far below the largest. The documented errors of the attention are those of fp32 arithmetic, with few rows
-for a weight times its V scale down to 2^-50 of the row's largest weight times the largest scale read."""
+far below the largest, scores past the range in which fp32 holds fractions. The documented errors of the
+attention are those of fp32 arithmetic, with few rows for a weight times its V scale down to 2^-50 of the
+row's largest weight times the largest scale read."""
 import numpy as np
 import pytest
 
@@ -115,3 +116,45 @@ def test_a_block_of_much_larger_values(hd, nh, nkv, r):
     want, tol = R.attention(q.astype(np.float64), kk[:, :300], vv[:, :300], 299)
     tol += floor_of(q, codes, sc, 299)
     assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / tol).max())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh,rows", [(2, 1), (8, 1), (4, 4)])
+@pytest.mark.parametrize("scale", [0x7bff, 0x3bff])
+def test_large_scores_with_full_mantissas(hd, nh, rows, scale):
+    """Scores of 1e4 and more, V scales with every bit of the mantissa set: finite, and inside the bounds."""
+    for seed in range(6):
+        rng = np.random.default_rng(100 * hd + 10 * nh + seed)
+        codes, sc = random_cache(rng, 3, 1, hd)
+        sc[1] = np.array([scale], np.uint16).view(np.float16)[0]
+        q = (rng.standard_normal((rows, nh, hd)) * 10.0 ** rng.uniform(3, 5)).astype(np.float32)
+        pos = 150 - rows
+        got = attend(q, codes, sc, pos)
+        kk, vv = values(codes, sc)
+        want, tol = R.attention(q.astype(np.float64), kk[:, :150], vv[:, :150], pos)
+        assert (np.abs(got - want) <= tol).all(), seed
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh,rows", [(2, 1), (8, 1), (4, 4)])
+@pytest.mark.parametrize("size", [3e5, 3e7, 1.7e9, 1e12, 1e30])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_scores_of_any_size(hd, nh, rows, size, sign):
+    """One dimension of q counts. Its best positions are two of equal score, all others far below them:
+    the output is the mean of the two values, however large the scores."""
+    rng = np.random.default_rng(hd + nh + rows)
+    codes, sc = random_cache(rng, 3, 1, hd)
+    sc[1] = np.array([0x3bff], np.uint16).view(np.float16)[0]
+    codes[0, ..., 0] = np.where(sign > 0, 2, 14)  # values of q's dimension: -6 d or 6 d, d = 1 ...
+    sc[0, ..., 0] = 1.0
+    a, b = 3, 77
+    for t in (a, b):
+        codes[0, t // 64, :, t % 64, 0] = 12  # ... but 4 d at the two
+    q = np.zeros((rows, nh, hd), np.float32)
+    q[..., 0] = sign * size * (1 + rng.random((rows, nh)))
+    if sign < 0:  # negative scores: the two are the least negative
+        codes[0, ..., 0] = np.where(codes[0, ..., 0] == 12, 9, 14)
+    got = attend(q, codes, sc, 150 - rows)
+    vv = values(codes, sc)[1][0]
+    want = np.broadcast_to((vv[a] + vv[b]) / 2, got.shape)
+    assert (np.abs(got - want) <= 2.0 ** -18 * np.abs(vv[[a, b]]).max(0)).all(), float(np.abs(got - want).max())

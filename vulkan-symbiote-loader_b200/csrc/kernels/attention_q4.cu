@@ -412,13 +412,14 @@ __global__ void __launch_bounds__(FQ_THREADS, FQ_CTAS_PER_SM) vsl_flash_decode_q
                 for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(x[i][j]));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 1));
             big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, 2));
-            // 2^-e with big * 2^-e in [1, 2) (the parts hold 2^13 times that, the codes' unit is 2^-9). Maxima
-            // below 2^-100, zero among them, take e = -100, so that no factor overflows.
+            // The parts hold q log2(e) / sqrt(hd) 2^(16 - e), below 2^15, with big * 2^-e in [1, 2). Maxima below 2^-100,
+            // zero among them, take e = -100, so that no factor overflows. What is left for the scores is a power
+            // of two (the codes' unit is 2^-9): score times q_mul is exact, and so no weight can come out above 1,
+            // and the largest as exactly 1, however large the scores.
             const int e = min(max((int)(__float_as_uint(big) >> 23), 27), 253) - 127;
-            const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-            const float up = p.scale * (1.4426950408889634f / 16.0f) * __uint_as_float((uint32_t)(127 + e) << 23);
+            const float up = __uint_as_float((uint32_t)(127 + e - 7) << 23);
             q_mul = make_float2(__shfl_sync(0xffffffffu, up, 8 * t4), __shfl_sync(0xffffffffu, up, 8 * t4 + 4));
-            const float scale = down * 8192.0f;
+            const float scale = p.scale * (1.4426950408889634f * 65536.0f) * __uint_as_float((uint32_t)(127 - e) << 23);
 #pragma unroll
             for (int i = 0; i < NB; i++)
 #pragma unroll
