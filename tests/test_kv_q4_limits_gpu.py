@@ -158,3 +158,28 @@ def test_scores_of_any_size(hd, nh, rows, size, sign):
     vv = values(codes, sc)[1][0]
     want = np.broadcast_to((vv[a] + vv[b]) / 2, got.shape)
     assert (np.abs(got - want) <= 2.0 ** -18 * np.abs(vv[[a, b]]).max(0)).all(), float(np.abs(got - want).max())
+
+
+# ---- rows enough for tiles of 128 columns ----
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("scale", [0x7bff, 0x3bff])
+def test_chunk_large_scores_with_full_mantissas(hd, scale):
+    rows, nh, pos = 16, 8, 134
+    for seed in range(6):
+        rng = np.random.default_rng(100 * hd + 10 * nh + seed)
+        codes, sc = random_cache(rng, 3, 1, hd)
+        sc[1] = np.array([scale], np.uint16).view(np.float16)[0]
+        q = (rng.standard_normal((rows, nh, hd)) * 10.0 ** rng.uniform(3, 5)).astype(np.float32)
+        got = attend(q, codes, sc, pos)
+        kk, vv = values(codes, sc)
+        want, tol = R.attention(q.astype(np.float64), kk[:, :150], vv[:, :150], pos)
+        # where the heaviest positions have code 8, the documented limit of 2^-50 shows
+        assert (np.abs(got - want) <= tol + floor_of(q, codes, sc, pos)).all(), seed
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("size", [3e5, 3e7, 1.7e9, 1e12, 1e30])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_chunk_scores_of_any_size(hd, size, sign):
+    test_scores_of_any_size(hd, 8, 16, size, sign)

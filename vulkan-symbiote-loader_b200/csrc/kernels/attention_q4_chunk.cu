@@ -367,7 +367,7 @@ __global__ void __launch_bounds__(FC_THREADS, 1) vsl_flash_chunk_q4_kernel(FqPar
                 r.codes[0] = r.codes[1];
                 r.scales[0] = r.scales[1];
             }
-            if (w == 0 && lane == 0) k_mul[i & 3] = valid ? p.scale * 1.4426950408889634f * fc_power(e - 21) : 0.0f;
+            if (w == 0 && lane == 0) k_mul[i & 3] = valid ? fc_power(e - 21) : 0.0f;
             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
             __syncwarp();
             if (lane == 0) mbar_arrive(&k_full[i & 1]);
@@ -498,7 +498,9 @@ __global__ void __launch_bounds__(FC_THREADS, 1) vsl_flash_chunk_q4_kernel(FqPar
     } else {
         // ================= softmax =================
         const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-        // ---- q: two parts of 2^13 q / 2^e, e from the row's largest magnitude, in the order of K ----
+        // ---- q: two parts of q log2(e) / sqrt(hd) 2^(16 - e), e from the row's largest magnitude, in the order of K.
+        // The factor left for the scores is a power of two: the product is exact, no exponent can come out above
+        // its row's maximum, however large the scores ----
         float q_mul;
         {
             // rows of q to shared memory, then a row half per thread
@@ -530,8 +532,8 @@ __global__ void __launch_bounds__(FC_THREADS, 1) vsl_flash_chunk_q4_kernel(FqPar
             big = fmaxf(big, red[0][hc ^ 1][t]);
             // maxima below 2^-100, zero among them, take e = -100, so that no factor overflows
             const int e = min(max((int)(__float_as_uint(big) >> 23), 27), 253) - 127;
-            const float down = fc_power(-e) * 8192.0f;
-            q_mul = fc_power(e) * (1.0f / 8192.0f);
+            const float down = p.scale * (1.4426950408889634f * 65536.0f) * fc_power(-e);
+            q_mul = fc_power(e - 16);
 #pragma unroll 1
             for (int k = 0; k < HALF / 16; k++) {  // rolled: straight code is slow the first time
                 float x[16];
@@ -577,7 +579,7 @@ __global__ void __launch_bounds__(FC_THREADS, 1) vsl_flash_chunk_q4_kernel(FqPar
                     fc_ld32(s_at, s);
                     mul = k_mul[i & 3];
                     if (mul == 0.0f) hi = 0;
-                    mul = fmaxf(mul * q_mul, 1.2e-38f);  // not zero: it meets infinities
+                    mul = fmaxf(mul * q_mul, fc_power(-126));  // not zero: it meets infinities
                     if (__any_sync(0xffffffffu, lo > 0 || hi < 32)) {
 #pragma unroll
                         for (int j = 0; j < 32; j++) s[j] = j >= lo && j < hi ? s[j] : -CUDART_INF_F;
@@ -600,8 +602,9 @@ __global__ void __launch_bounds__(FC_THREADS, 1) vsl_flash_chunk_q4_kernel(FqPar
             if (i > 0) ok = mbar_wait(&o_full[(i - 1) & 1], (uint32_t)(((i - 1) >> 1) & 1)) && !*aborted;
             ok = __all_sync(0xffffffffu, ok);
             if (i < n) {
-                // exp2(s mul - m + 15)
-                const float2 mul2x = make_float2(mul, mul), off = make_float2(15.0f - m0, 15.0f - m0);
+                // exp2(s mul - m + 15); 15 - m rounded down, so that it is at most 2^15 and, -m being a float, at least 1
+                // for the largest
+                const float2 mul2x = make_float2(mul, mul), off = make_float2(__fsub_rd(15.0f, m0), __fsub_rd(15.0f, m0));
                 float2 sum = make_float2(0.0f, 0.0f);
                 const bool whole = __all_sync(0xffffffffu, lo <= 0 && hi >= 32);
 #pragma unroll 1
