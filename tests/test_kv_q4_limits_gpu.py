@@ -1,7 +1,7 @@
 """4-bit KV cache on the GPU at the ends of its ranges: padding rows whatever the norm, weights and values
-far below the largest, scores past the range in which fp32 holds fractions. The documented errors of the
-attention are those of fp32 arithmetic, with few rows for a weight times its V scale down to 2^-50 of the
-row's largest weight times the largest scale read."""
+far below the largest, scores past the range in which fp32 holds fractions, scales that are not finite.
+The documented errors of the attention are those of fp32 arithmetic, with few rows for a weight times its
+V scale down to 2^-50 of the row's largest weight times the largest scale read."""
 import numpy as np
 import pytest
 
@@ -158,6 +158,28 @@ def test_scores_of_any_size(hd, nh, rows, size, sign):
     vv = values(codes, sc)[1][0]
     want = np.broadcast_to((vv[a] + vv[b]) / 2, got.shape)
     assert (np.abs(got - want) <= 2.0 ** -18 * np.abs(vv[[a, b]]).max(0)).all(), float(np.abs(got - want).max())
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh,nkv", [(2, 2), (8, 2), (8, 1)])
+@pytest.mark.parametrize("bad", [np.nan, np.inf, -np.inf])
+@pytest.mark.parametrize("n", [20, 300])
+def test_a_scale_that_is_not_finite_leaves_the_other_blocks_alone(hd, nh, nkv, bad, n):
+    """Small scales beside it keep their digits."""
+    rng = np.random.default_rng(hd + nh + nkv)
+    codes, sc = random_cache(rng, 5, nkv, hd, k_scale=0.02, v_scale=2.0 ** -21)
+    codes[1, 0, :, 9, 32:64] = 8 + rng.integers(1, 8, 32)  # no code 8: times an infinity that is NaN as well
+    sc[1, 0, :, 9, 1] = bad
+    q = rng.standard_normal((1, nh, hd)).astype(np.float32)
+    got = attend(q, codes, sc, n - 1)
+    assert not np.isfinite(got[..., 32:64]).any()
+    clean = sc.copy()
+    clean[1, 0, :, 9, 1] = 0
+    kk, vv = values(codes, clean)
+    want, tol = R.attention(q.astype(np.float64), kk[:, :n], vv[:, :n], n - 1)
+    tol += floor_of(q, codes, clean, n - 1)
+    rest = [d for d in range(hd) if not 32 <= d < 64]
+    assert (np.abs(got - want) <= tol)[..., rest].all(), float((np.abs(got - want) / tol)[..., rest].max())
 
 
 # ---- rows enough for tiles of 128 columns ----

@@ -569,9 +569,23 @@ __global__ void __launch_bounds__(FQ_THREADS, FQ_CTAS_PER_SM) vsl_flash_decode_q
 #pragma unroll
             for (int i = 1; i < 4 * T; i++) m_new = make_float2(fmaxf(m_new.x, s[i].x), fmaxf(m_new.y, s[i].y));
             // fp16 exponent field e: scales below 2^(e - 14); e = 0 for zeros and subnormals
-            const uint32_t need = (top >> 10) + 113u;  // 127 - 14
+            uint32_t need = (top >> 10) + 113u;  // 127 - 14
             if (__any_sync(0xffffffffu, m_new.x * q_mul.x > mc.x || m_new.y * q_mul.y > mc.y ||
                                             need > d_exp)) {
+                // A scale that is not finite does not count, or the other blocks would lose digits with it. Lanes whose
+                // position no column sees have top = 0.
+                if (__any_sync(0xffffffffu, top >= 0x7c00u)) {
+                    uint32_t finite = 113u;
+#pragma unroll
+                    for (int i = 0; i < T; i++)
+#pragma unroll
+                        for (int j = 0; j < NB; j++) {
+                            const unsigned char* vs = ring + i * STAGE_BYTES + 2 * CODE_BYTES + SCALE_BYTES;
+                            const uint32_t e = *reinterpret_cast<const uint16_t*>(vs + lane * (2 * NB) + 2 * j) >> 10 & 31u;
+                            finite = max(finite, e < 31u ? e + 113u : 0u);
+                        }
+                    if (top >= 0x7c00u) need = finite;
+                }
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) {
                     m_new.x = fmaxf(m_new.x, __shfl_xor_sync(0xffffffffu, m_new.x, d));
