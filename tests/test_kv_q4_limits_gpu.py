@@ -182,6 +182,23 @@ def test_a_scale_that_is_not_finite_leaves_the_other_blocks_alone(hd, nh, nkv, b
     assert (np.abs(got - want) <= tol)[..., rest].all(), float((np.abs(got - want) / tol)[..., rest].max())
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("nh,rows", [(2, 1), (8, 1), (8, 16)])
+@pytest.mark.parametrize("n", [20, 150])
+def test_scores_past_the_range_of_fp32_are_no_zeros(hd, nh, rows, n):
+    """Finite queries whose scores overflow: NaN, as for infinite ones, and only in their head."""
+    rng = np.random.default_rng(hd + nh + rows)
+    codes, sc = random_cache(rng, 3, 1, hd)
+    codes[0, ..., 0], sc[0, ..., 0] = 12, 8.0
+    q = rng.standard_normal((rows, nh, hd)).astype(np.float32)
+    fine = attend(q, codes, sc, n - rows)
+    q[0, 1], q[0, 1, 0] = 0.0, 3e38
+    got = attend(q, codes, sc, n - rows)
+    keep = np.ones((rows, nh), bool)
+    keep[0, 1] = False
+    assert np.isfinite(fine).all() and np.isnan(got[0, 1]).all() and np.array_equal(got[keep], fine[keep])
+
+
 # ---- rows enough for tiles of 128 columns ----
 
 @pytest.mark.parametrize("hd", [64, 128])

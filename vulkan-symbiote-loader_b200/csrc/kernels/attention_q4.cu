@@ -738,7 +738,8 @@ __global__ void __launch_bounds__(FQ_THREADS, FQ_CTAS_PER_SM) vsl_flash_decode_q
         for (int j = 0; j < 2; j++) {
             const int col = 2 * t4 + j;
             if (col >= cols) continue;
-            const float lj = j ? l.y : l.x, w = lj == 0.0f ? 0.0f : f / lj;  // a row that sees nothing gives zeros
+            // a row that sees nothing gives zeros; without weights because its scores overflowed, NaN
+            const float lj = j ? l.y : l.x, w = lj == 0.0f && (j ? mc.y : mc.x) == -CUDART_INF_F ? 0.0f : f / lj;
             float* dst = fq_out(p, b, g, c, col, HD);
 #pragma unroll
             for (int i = 0; i < NB; i++)
