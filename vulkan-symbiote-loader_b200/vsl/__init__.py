@@ -199,17 +199,18 @@ def check(rc: int):
 
 def _ptr(x):
     """Device/host pointer of a torch tensor, numpy array, int or None."""
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     try:  # a tensor, the usual case on the path of a decode step
         return x.data_ptr()
     except AttributeError:
         pass
     if isinstance(x, int):
-        return x
-    if hasattr(x, "ctypes"):
+        return int(x)
+    try:
         return x.ctypes.data
-    raise TypeError(f"cannot take a pointer of {type(x)}")
+    except AttributeError:
+        raise TypeError(f"cannot take a pointer of {type(x)}") from None
 
 
 # ---------------------------------------------------------------------------------------
