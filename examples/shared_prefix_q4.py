@@ -18,7 +18,7 @@ import vsl  # noqa: E402
 
 CONFIG = dict(n_layers=4, d_model=512, n_heads=8, n_kv=2, head_dim=64, ffn=1376, vocab=4096, rope_theta=10000.0,
               eps=1e-5)
-CHUNK = 16  # prompt rows per pass (vsl_gemv takes up to 16)
+CHUNK = 16  # prompt rows, or sequences of a step, per pass (vsl_gemv takes up to 16)
 
 
 class Decoder:
@@ -55,9 +55,9 @@ class Decoder:
         self.kv = vsl.KvPages(self.table, n_seq, self.max_pages, page, self.ref, n_pages, list(self.pools), page_bytes,
                               lens=self.lens)
         self.page_ws = torch.zeros(vsl.kv_pages_workspace_size(n_seq, n_pages), dtype=torch.uint8, **dev)
-        self.attn_ws = torch.zeros(max(vsl.flash_decode_q4_workspace_size(1, CHUNK, nh, nkv, hd),
-                                       vsl.flash_decode_q4_workspace_size(n_seq, 1, nh, nkv, hd)), dtype=torch.uint8,
-                                   **dev)
+        ws = max(vsl.flash_decode_q4_workspace_size(1, CHUNK, nh, nkv, hd),
+                 vsl.flash_decode_q4_workspace_size(min(n_seq, CHUNK), 1, nh, nkv, hd))
+        self.attn_ws = torch.zeros(ws, dtype=torch.uint8, **dev)
         ang = torch.arange(max_seq, dtype=torch.float64, **dev)[:, None] * c["rope_theta"] ** (
             -torch.arange(0, hd, 2, dtype=torch.float64, **dev) / hd)
         self.cos, self.sin = ang.cos().float(), ang.sin().float()
@@ -126,10 +126,19 @@ class Decoder:
         return logits[-1]
 
     def step(self, ids, seqs):
-        """One token for each sequence in seqs; their logits."""
+        """One token for each sequence in seqs (one at least); their logits."""
         self.extend(seqs, 1)
-        seq = self._ints(seqs)
-        return self.forward(self._ints(ids), seq, (self.lens[seq.long()] - 1).contiguous(), len(seqs), 1)
+        logits = []
+        for at in range(0, len(seqs), CHUNK):
+            seq = self._ints(seqs[at:at + CHUNK])
+            logits.append(self.forward(self._ints(ids[at:at + CHUNK]), seq, (self.lens[seq.long()] - 1).contiguous(),
+                                       len(seq), 1))
+        return torch.cat(logits)
+
+    def check(self):
+        """Raises what the kernels reported: a pool that ran out of pages, positions past the cache."""
+        if self.status.item():
+            raise RuntimeError("device status %d" % self.status.item())
 
 
 def answers(dec, prompt, n, tokens, share=True):
@@ -156,19 +165,24 @@ def main(argv=None):
     ap.add_argument("--answers", type=int, default=6)
     ap.add_argument("--tokens", type=int, default=24)
     a = ap.parse_args(argv)
-    dec = Decoder(n_seq=a.answers, max_seq=a.prompt + a.tokens, n_pages=64 + 4 * a.answers)
+    if min(a.prompt, a.answers, a.tokens) < 1 or a.answers > CONFIG["vocab"]:
+        ap.error("--prompt, --answers and --tokens are at least 1, --answers at most %d" % CONFIG["vocab"])
+    page = 64  # pages: the prompt's once, and for every answer its last one and those of its tokens
+    dec = Decoder(n_seq=a.answers, max_seq=a.prompt + a.tokens, page=page,
+                  n_pages=-(-a.prompt // page) + a.answers * (2 + a.tokens // page))
     prompt = [(i * 2654435761 >> 7) % CONFIG["vocab"] for i in range(a.prompt)]
     got, _ = answers(dec, prompt, a.answers, a.tokens)
+    dec.check()
     for i, ids in enumerate(got):
         print("answer %d: %s" % (i, ids))
     unshared = a.answers * -(-(a.prompt + a.tokens - 1) // dec.page)
     print("pages in use: %d shared, %d unshared" % (dec.pages_in_use(), unshared))
     dec.free(list(range(0, a.answers, 2)))
     print("after freeing every other answer: %d in use, %d moved" % dec.compact())
-    lg = dec.step([ids[-1] for ids in got[1::2]], list(range(1, a.answers, 2)))
-    print("next tokens of the others: %s" % lg.argmax(-1).tolist())
-    if dec.status.item():
-        raise RuntimeError("device status %d" % dec.status.item())
+    if a.answers > 1:
+        lg = dec.step([ids[-1] for ids in got[1::2]], list(range(1, a.answers, 2)))
+        dec.check()
+        print("next tokens of the others: %s" % lg.argmax(-1).tolist())
 
 
 if __name__ == "__main__":

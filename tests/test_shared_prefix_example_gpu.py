@@ -47,3 +47,41 @@ def test_example_runs(capsys):
     E.main(["--prompt", "70", "--answers", "3", "--tokens", "4"])
     out = capsys.readouterr().out
     assert "pages in use" in out and "next tokens" in out
+
+
+@pytest.mark.parametrize("prompt,n,tokens", [(70, 1, 3), (5, 1, 1), (130, 37, 3), (4600, 2, 2), (64, 3, 130)])
+def test_example_takes_any_size(capsys, prompt, n, tokens):
+    """One answer, more answers than rows of a pass, prompts and answers of many pages."""
+    E.main(["--prompt", str(prompt), "--answers", str(n), "--tokens", str(tokens)])
+    lines = capsys.readouterr().out.splitlines()
+    assert [x.split(":")[0] for x in lines[:n]] == ["answer %d" % i for i in range(n)]
+    assert ("next tokens" in lines[-1]) == (n > 1)
+
+
+def test_steps_in_groups_are_those_of_each_group():
+    prompt = [(5 * i + 1) % E.CONFIG["vocab"] for i in range(70)]
+    n = E.CHUNK + 3
+    decs = [E.Decoder(n_seq=n, max_seq=90, n_pages=48) for _ in range(2)]
+    ids = [(11 * i) % E.CONFIG["vocab"] for i in range(n)]
+    for d in decs:
+        d.prompt(prompt, 0)
+        d.fork(0, list(range(1, n)))
+    whole = decs[0].step(ids, list(range(n)))
+    parts = [decs[1].step(ids[a:b], list(range(a, b))) for a, b in ((0, E.CHUNK), (E.CHUNK, n))]
+    assert torch.equal(whole, torch.cat(parts))
+    for d in decs:
+        d.check()
+
+
+@pytest.mark.parametrize("args", [["--answers", "0"], ["--prompt", "0"], ["--tokens", "0"], ["--answers", "5000"]])
+def test_example_refuses_sizes_that_are_none(capsys, args):
+    with pytest.raises(SystemExit):
+        E.main(args)
+    assert "at least 1" in capsys.readouterr().err
+
+
+def test_a_pool_that_runs_out_is_reported():
+    dec = E.Decoder(n_seq=2, max_seq=256, n_pages=2)
+    dec.prompt(list(range(200)), 0)
+    with pytest.raises(RuntimeError):
+        dec.check()
