@@ -295,7 +295,8 @@ VSL_API int vsl_kv_pages_workspace_size(int n_seq, int n_pages, size_t* bytes);
 /* Sequence dst[k] becomes a copy of src[k]: the pages it held are given back, it shares src's whole
  * pages, and an unfinished last page is copied to a new page. A target is the source or target of no
  * other fork of the call (such a fork, and one whose source is longer than its table row, is left out
- * with VSL_ERR_BOUNDS). A fork that finds no page leaves its target empty. Three launches. */
+ * with VSL_ERR_BOUNDS). Entries of src that name no page are copied as they are (VSL_ERR_BOUNDS). A fork that
+ * finds no page leaves its target empty. Three launches. */
 VSL_API int vsl_kv_fork(const vsl_kv_pages* kv, const int32_t* src, const int32_t* dst, int n, void* workspace,
                         size_t workspace_bytes, int* status, void* stream);
 

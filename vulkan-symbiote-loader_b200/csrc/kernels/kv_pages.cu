@@ -173,9 +173,10 @@ __global__ void __launch_bounds__(KP_THREADS) vsl_kv_fork_kernel(KpParams p, con
     const int s = src[k], d = dst[k], f = fresh[k], len = max(p.lens[s], 0);
     const int full = f == -2 ? 0 : min(len / p.page_size, p.max_pages);  // whole pages to share
     const int tail = f >= 0 && full < p.max_pages ? p.table[(size_t)s * p.max_pages + full] : -1;
+    const bool has_tail = tail >= 0 && tail < p.n_pages;  // else there is nothing to copy: f stays free, the entry is the source's
     if (blockIdx.x == 0 && blockIdx.y == 0) {
         for (int i = threadIdx.x; i < p.max_pages; i += KP_THREADS) {
-            int pg = i < full ? p.table[(size_t)s * p.max_pages + i] : i == full && f >= 0 ? f : -1;
+            int pg = i < full ? p.table[(size_t)s * p.max_pages + i] : i == full && f >= 0 ? (has_tail ? f : tail) : -1;
             if (i < full) {
                 if (pg >= 0 && pg < p.n_pages) atomicAdd(p.ref + pg, 1);
                 else set_status(p.status, VSL_ERR_BOUNDS);
@@ -183,12 +184,12 @@ __global__ void __launch_bounds__(KP_THREADS) vsl_kv_fork_kernel(KpParams p, con
             p.table[(size_t)d * p.max_pages + i] = pg;
         }
         if (threadIdx.x == 0) {
-            if (f >= 0) p.ref[f] = 1;
+            if (has_tail) p.ref[f] = 1;
             p.lens[d] = f == -2 ? 0 : len;
         }
     }
     if (f < 0) return;
-    if (tail < 0 || tail >= p.n_pages) {
+    if (!has_tail) {
         if (threadIdx.x == 0) set_status(p.status, VSL_ERR_BOUNDS);
         return;
     }
