@@ -14,13 +14,14 @@
 //   - Both products have the exact integers n - 8 as the 16-row operand (rows: positions for the
 //     scores, dimensions for the output): a shift, and a mask and a multiply-add per pair of codes, give
 //     eight of them (the pairs sit in the words in the order the fragments want). Products of
-//     codes alone (the offset subtracted from the sums) save the multiply-adds (42.3 against 43.5 us), but
+//     codes alone (the offset subtracted from the sums) save the multiply-adds (3 % of the time), but
 //     not the accuracy: errors 1.5 to 4 times those of a plain fp32 form.
 //   - The scales stay in fp32: a block's partial scores are multiplied by its d, and p_t is multiplied
 //     by d_t of each V block before the second product.
-//   - The other operand, q or p d, is split into two fp16 values (22 bits). With at most four
-//     (row, head) columns the parts are the two halves of the eight operand columns, so that one
-//     instruction covers both; with up to eight they are two instructions.
+//   - The other operand, q (times log2(e) / sqrt(hd)) or p d, is split into two fp16 values (22 bits), the
+//     low one of p d 2^11 times as large. With at most four (row, head) columns the parts are the two
+//     halves of the eight operand columns, so that one instruction covers both; with up to eight they are
+//     two instructions.
 //   - Scores come out by (position, two columns) per lane, with a column's statistics in the lanes that
 //     hold its outputs; movmatrix turns p d into the operand of the second product.
 //
@@ -35,8 +36,8 @@
 //
 // Twelve warps of 168 registers per SM: 16 of 128 take as long, 10 a sixth longer. Measured on a B200:
 // 16 sequences of 8192 positions, 32 / 8 heads of 128: 44.5 us (3.4 TB/s, 53 % of the measured copy
-// rate; 4.7 TB/s without the start and the joins, 11 us); 131071 positions of one sequence 46.6 us; 384
-// positions of 32 heads 7.3 us. The loop issues 650 instructions
+// rate; 4.6 TB/s in the slope from 8192 to 24576 positions, so 12 us of start and joins); 131071 positions of
+// one sequence 46.4 to 47.2 us; 384 positions of 32 heads 7.2 us. The loop issues 670 instructions
 // per stage at two thirds of the SM's issue rate: that bounds it.
 #include <cuda_runtime.h>
 #include <math_constants.h>
@@ -61,14 +62,16 @@ constexpr int FQ_MAX_BATCH = 1024;
 // Stages after which a warp's accumulators move to its place in the workspace. The matrix unit cuts
 // its sums instead of rounding them, about 2^-26 of the sum per instruction and always towards zero, so a
 // chain of instructions stays short whatever the length. Twice / four times as long (head_dim 128 / 64):
-// 1 to 2 % faster, errors 1.4e-6 instead of 0.9e-6 / 0.7e-6 where a plain fp32 form has 1.2e-6 / 0.8e-6.
+// 1 to 2 % faster, errors 1.4e-6 instead of 0.9e-6 / 0.7e-6 where a plain fp32 form has 1.2e-6 / 0.8e-6 (measured
+// with a low part of p d that was cut; rounded, the errors are 0.6e-6 to 0.7e-6 at head_dim 128).
 template <int HD, bool SPLIT_N>
 __host__ __device__ constexpr int fq_chain() {
     return (SPLIT_N ? 16 : 8) / (HD == 64 ? 2 : 1);
 }
 // Stages a warp processes at once, of two such groups in its ring: two spread a group's fixed chain
-// (wait, maxima, exponentials) over twice the positions (5.05 against 4.72 TB/s in long runs); with eight columns of 128 dimensions the
-// registers hold one.
+// (wait, maxima, exponentials) over twice the positions (7 % faster in long runs); with eight columns of 128
+// dimensions the registers hold one. Slopes in long runs of 32 heads over 8: 4.6 TB/s, 4.0 at head_dim 64; of 64
+// heads 3.1 and 2.9 TB/s.
 template <int HD, bool SPLIT_N>
 __host__ __device__ constexpr int fq_group() {
     return SPLIT_N || HD == 64 ? 2 : 1;
@@ -219,7 +222,7 @@ __global__ void __launch_bounds__(FQ_THREADS, FQ_CTAS_PER_SM) vsl_flash_decode_q
     // Stages per part from the stages of all items and of the longest: ceil(s / q) parts of each item
     // of s stages are at most as many as there are workers. A CTA per item needs no join between CTAs,
     // which costs about as much as a stage: with q + 4 instead of q + 1 below, 4 x 2048 positions of 8 KV heads
-    // take 15.4 us against 11.8, 8 x 2048 15.5 against 14.0; with q + 2, 16 x 8192 43.9 against 43.5.
+    // took 15.4 us against 11.8, 8 x 2048 15.5 against 14.0; with q + 2, 16 x 8192 took 1 % more.
     auto plan = [&](uint32_t total, uint32_t most, bool& cta_items) {
         const unsigned long long all = (unsigned long long)total * items_per_seq;
         const uint32_t room = workers - items;
@@ -933,10 +936,10 @@ int flash_decode_q4_impl(const float* q, const void* k_cache, const void* v_cach
     if ((double)B * n_kv * p.tiles * units > 2e9)
         return set_error(VSL_ERR_UNSUPPORTED, "flash_decode_q4: %d sequences x %d KV heads x %d column tiles over %lld "
                          "positions is too much for one call", B, n_kv, p.tiles, (long long)max_pages * page_size);
-    // From 48 columns per KV head on (80 at head_dim 64) unpacking once for all of them is faster. Columns: this
-    // form / the other, in us: 32 / 8 heads of 128, 16 x 2048 positions: 32: 64 / 83, 48: 128 / 72, 128: 315 / 76;
-    // 1 x 2048: 32: 15.7 / 18.5, 48: 16.0 / 16.7, 128: 22.1 / 20.2, 512: 63 / 28; head_dim 64, 4 x 4000: 64: 35 / 40,
-    // 96: 53 / 36.
+    // From 48 columns per KV head on (80 at head_dim 64) the form for many rows, which unpacks once for all of them,
+    // is faster. Few rows / many rows, in us, by columns: 32 / 8 heads of 128, 16 x 2048 positions: 32: 65.6 / 83,
+    // 48: 128 / 75, 128: 315 / 80; 1 x 2048: 32: 15.4 / 18.5, 48: 16.0 / 16.0, 128: 22.1 / 19.8, 512: 63 / 28.5;
+    // head_dim 64, 4 x 4000: 64: 36.2 / 40, 96: 53 / 35.7.
     if ((long long)rows * p.G >= (head_dim == 128 ? 48 : 80)) return fc_launch(p, head_dim, st);
     const int grid = fq_grid((long long)B * n_kv * p.tiles * units);
     const bool few = rows * p.G <= FQ_COLS / 2;

@@ -109,9 +109,11 @@ __device__ __forceinline__ void q4_codes(const float (*x)[4], uint32_t* codes, _
 // lane group handles HEADS heads of one row: their loads are all requested first, beside the chain
 // position -> page, and the row's rotation factors are read once.
 // Measured on a B200: 8192 rows of 32 / 8 heads of 128 into the 4-bit cache 75 us (4.6 TB/s, 71 % of the
-// measured copy rate; 213 us with one head per group and its load behind the page), into the fp16 cache
-// without norm and rotation 62 us (5.9 TB/s, 92 %): the difference is the arithmetic of the codes. A
-// decode step takes 2.8 us, which is the launch and the chain position -> page -> store.
+// measured copy rate; 213 us with one head per group and its load behind the page), fp16 65 us (5.7 TB/s),
+// fp32 70 us (5.8 TB/s). Without norm and rotation 65, 61 and 66 us. So of the 4-bit cache's 75 us the codes
+// take about 10 (against fp16, which stores 24 MB more), the norm 6, the rotation 4; the warps wait for their
+// loads first (3.1 per issue), then for fixed latencies (2.1), with three quarters of the issue slots
+// used. A decode step takes 2.8 us, which is the launch and the chain position -> page -> store.
 template <int HD, int KVDT, int HEADS>
 __global__ void __launch_bounds__(KA_THREADS) vsl_kv_append_kernel(KvAppendParams p) {
     constexpr int L = HD / 4, NB = HD / 32;
@@ -278,7 +280,8 @@ struct KvReadParams {
 // A lane group handles HEADS of a row's 2 n_kv K and V heads, all loads first. fp32 / fp16: four
 // dimensions per lane. 4-bit: 8 lanes, head_dim / 16 bytes of codes each; a lane's run of K holds 8
 // neighbouring dimensions of each of NB / 2 blocks, a run of V 4 of each of NB blocks. 8192 positions
-// of 8 heads of 128 to fp16: 11 us (3.9 TB/s; 17 us with one 2-byte piece per lane).
+// of 8 heads of 128 to fp16: 11 us (3.9 TB/s; 17 us with one 2-byte piece per lane; 16 rows take 2.1), of an
+// fp16 cache 13.4 us (5.0 TB/s), of an fp32 cache to fp32 23.4 us (5.7 TB/s).
 template <int HD, int KVDT, typename OT, int HEADS>
 __global__ void __launch_bounds__(KA_THREADS) vsl_kv_read_kernel(KvReadParams p) {
     constexpr bool Q4 = KVDT == VSL_Q4_0;
